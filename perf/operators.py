@@ -37,8 +37,8 @@ def listed():
         {"name": "product one token", "op": "product", "rows": 1, "cols": 4096, "inner": 2048, "out": "bf16"},
         # a small odd batch against a long inner size
         {"name": "product small batch", "op": "product", "rows": 33, "cols": 2048, "inner": 8192, "out": "bf16"},
-        # nothing is a multiple of a tile: rows, columns and an inner size that ends inside a block of 128; fp16 output
-        {"name": "product ragged fp16 out", "op": "product", "rows": 517, "cols": 1001, "inner": 2056, "out": "fp16"},
+        # nothing is a multiple of a tile: rows, columns and an inner size that ends inside a block of 128; 32-bit output
+        {"name": "product ragged fp32 out", "op": "product", "rows": 517, "cols": 1001, "inner": 2056, "out": "fp32"},
         # a prompt of 8192 tokens, wide layer: matrix rate
         {"name": "product long prompt", "op": "product", "rows": 8192, "cols": 8192, "inner": 8192, "out": "bf16"},
         # one token's 8 experts of 64: the chosen experts' weights once
@@ -70,7 +70,7 @@ def draw(rng):
         return case
     if op == "product":
         return {"op": op, "rows": _log(rng, 1, 8192), "cols": _size(rng, 64, 8192), "inner": _size(rng, 64, 8192),
-                "out": rng.choice(["bf16", "bf16", "fp16"])}
+                "out": rng.choice(["bf16", "bf16", "fp16", "fp32"])}
     experts = _log(rng, 2, 64)
     case = {"op": op, "tokens": _log(rng, 1, 8192), "topk": rng.randint(1, min(8, experts)), "experts": experts,
             "cols": _size(rng, 64, 4096), "inner": _size(rng, 64, 4096) // 8 * 8, "type": rng.choice(["fp8", "fp8", "bf16", "fp16"]),
