@@ -11,7 +11,8 @@
 // Precision of the e4m3 MFMAs (both f8f6f4 and the older 16x16x32 form, measured with single products): 8 consecutive products
 // are aligned to the one of largest exponent E and cut below 2^(E - 13); the groups of 8 are then added with 24 bits.  For normal
 // operands that is 1.4e-5 of the result (2-norm), for heavy-tailed ones 5e-5: far inside a bf16 or fp16 rounding, but not a 32-bit
-// result, so the 8-bit products have no fp32 output.  (Converting to bf16 first would be exact and half the matrix rate.)
+// result.  For fp32 outputs (KIND_FP8_WIDE) the operands become bf16 in registers, which is exact, and a block is four v_mfma_f32_16x16x32_bf16:
+// those keep 24 bits below the largest of 8 products (2^16 - 2^16 + 2^j keeps 2^j down to j = -8 in one group of 8), at half the matrix rate.
 //
 // matmul_kernel: tile BM rows x BN weight rows, both operands through LDS by LDS-DMA (16 bytes per lane, S stages of one K step).  LDS
 // rows are 128 B; the 16-byte chunk index is XOR-swizzled on the source address so that the 16 rows x 4 chunks of a fragment read fall
@@ -42,7 +43,8 @@ __device__ __forceinline__ buffer_t make_buffer(const char* base) {
 }
 #endif
 
-enum { KIND_FP8 = 0, KIND_BF16 = 1, KIND_FP16 = 2 };
+enum { KIND_FP8 = 0, KIND_BF16 = 1, KIND_FP16 = 2, KIND_FP8_WIDE = 3 };
+constexpr bool scaled(int kind) { return kind == KIND_FP8 || kind == KIND_FP8_WIDE; }
 
 struct MatmulParams {
   const char* x;
@@ -75,6 +77,27 @@ __device__ __forceinline__ f32x4 mfma_step(const i32x8& a, const i32x8& b, f32x4
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a1), __builtin_bit_cast(f16x8, b1), c, 0, 0, 0);
     }
   }
+}
+// 32 e4m3 values as bf16, and a K step of a 16 x 16 tile on two such operands
+struct Wide {
+  bf16x8 v[4];
+};
+__device__ __forceinline__ Wide widen(const i32x8& a) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  Wide r;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[d], 1.f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[d], 1.f, true);
+    bf16x8& t = r.v[d >> 1];
+    t[4 * (d & 1)] = lo[0], t[4 * (d & 1) + 1] = lo[1], t[4 * (d & 1) + 2] = hi[0], t[4 * (d & 1) + 3] = hi[1];
+  }
+  return r;
+}
+__device__ __forceinline__ f32x4 mfma_wide(const Wide& a, const Wide& b) {
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
+  return c;
 }
 template <typename V>
 __device__ __forceinline__ i32x8 join_pair(const V& lo, const V& hi) {
@@ -210,9 +233,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void matmul_kernel(MatmulParams p) 
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "every wave fills the same number of rows");
   static_assert(BM % 64 == 0 && BM / 64 < NW, "a wave loads 64 row scales or the weight scales");
   constexpr int SCALES = (BM + BN) * 128;                  // in a stage: x rows, w rows, x scales, w scales
-  constexpr int STAGE = SCALES + (KIND == KIND_FP8 ? NW * 256 : 0);
+  constexpr int STAGE = SCALES + (scaled(KIND) ? NW * 256 : 0);
   __shared__ __attribute__((aligned(1024))) char smem[S * STAGE];
-  constexpr int PIECES = XI + WI + (KIND == KIND_FP8);     // LDS-DMA instructions of a wave per stage
+  constexpr int PIECES = XI + WI + scaled(KIND);     // LDS-DMA instructions of a wave per stage
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int fr = lane & 15, fg = lane >> 4;
@@ -246,7 +269,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void matmul_kernel(MatmulParams p) 
   // scales, one 4-byte piece per lane: waves v < BM / 64 load those of rows 64 v ..., the others (all alike) one per 64 weight rows
   const float* ssrc = nullptr;
   int64_t sstep = 0;
-  if constexpr (KIND == KIND_FP8) {
+  if constexpr (scaled(KIND)) {
     const int nb = (p.N + 127) >> 7;
     const bool of_rows = wave < BM / 64;
     ssrc = of_rows ? p.xs + source_row(wave * 64 + lane) * p.xs_m
@@ -262,7 +285,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void matmul_kernel(MatmulParams p) 
 #pragma unroll
     for (int i = 0; i < XI; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(xtile, (lds_ptr)(s + i * NW * 1024), 16, PART ? (xin ? xoff[i] + k0 : xoff[i] - xchunk) : xoff[i], PART ? 0 : k0, 0, 0);
-    if constexpr (KIND == KIND_FP8) __builtin_amdgcn_global_load_lds((gbl_ptr)(ssrc + kb * sstep), (lds_ptr)(smem + st + SCALES + wave * 256), 4, 0, 0);
+    if constexpr (scaled(KIND)) __builtin_amdgcn_global_load_lds((gbl_ptr)(ssrc + kb * sstep), (lds_ptr)(smem + st + SCALES + wave * 256), 4, 0, 0);
   };
   auto fill_w = [&](int kb, int st, auto part) {
     constexpr bool PART = decltype(part)::value;
@@ -299,6 +322,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void matmul_kernel(MatmulParams p) 
   const int wofs[2] = {(fg ^ swz_w(wrow)) * 16, ((fg + 4) ^ swz_w(wrow)) * 16};
   const int xofs[2] = {(fg ^ swz_x(fr)) * 16, ((fg + 4) ^ swz_x(fr)) * 16};
   i32x8 w[TN], x[2];
+  Wide ww[TN], xw;                                         // (KIND_FP8_WIDE)
   f32x4 part[2];
   float sx[2], s[2] = {0.f, 0.f}, sw = 0.f;
   auto read_w = [&](int st, int f) {
@@ -307,18 +331,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void matmul_kernel(MatmulParams p) 
   };
   auto read_x = [&](int st, int i, int slot) {
     x[slot] = read_pair(xbase + st + i * 2048 + xofs[0], xbase + st + i * 2048 + xofs[1]);
-    if constexpr (KIND == KIND_FP8) sx[slot] = *reinterpret_cast<const float*>(smem + st + SCALES + ((wm * TM + i) * 16 + fr) * 4);
+    if constexpr (scaled(KIND)) sx[slot] = *reinterpret_cast<const float*>(smem + st + SCALES + ((wm * TM + i) * 16 + fr) * 4);
   };
   auto read_sw = [&](int st) {
-    return KIND == KIND_FP8 ? *reinterpret_cast<const float*>(smem + st + SCALES + BM * 4 + wn * 4) : 0.f;
+    return scaled(KIND) ? *reinterpret_cast<const float*>(smem + st + SCALES + BM * 4 + wn * 4) : 0.f;
   };
   // MFMA number n = i * TN + f of a step, and the FMAs that add the partial result of number n (by its block's scale)
   auto multiply = [&](int i, int f) {
-    if constexpr (KIND == KIND_FP8) part[f & 1] = mfma_step<KIND>(w[f], x[i & 1], f32x4{0.f, 0.f, 0.f, 0.f});
-    else acc[i][f] = mfma_step<KIND>(w[f], x[i & 1], acc[i][f]);
+    if constexpr (KIND == KIND_FP8) {
+      part[f & 1] = mfma_step<KIND>(w[f], x[i & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+    } else if constexpr (KIND == KIND_FP8_WIDE) {          // (a step's weights are widened once, a row fragment before its first use)
+      if (i == 0) ww[f] = widen(w[f]);
+      if (f == 0) xw = widen(x[i & 1]);
+      part[f & 1] = mfma_wide(ww[f], xw);
+    } else acc[i][f] = mfma_step<KIND>(w[f], x[i & 1], acc[i][f]);
   };
   auto promote = [&](int i, int f) {
-    if constexpr (KIND == KIND_FP8) {
+    if constexpr (scaled(KIND)) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[i][f][q] = fmaf(part[f & 1][q], s[i & 1], acc[i][f][q]);
     }
@@ -478,7 +507,7 @@ __global__ __launch_bounds__(512, 2) void matmul_few_kernel(MatmulParams p) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int NW = 8, BM = 8 * XG, BN = 16 * NT, MT = (XG + 1) / 2, WG = 2 * NT;
   constexpr int SCALES = (2 * MT + WG) * 1024;             // in a stage: x rows, w rows, scales
-  constexpr int STAGE = SCALES + (KIND == KIND_FP8 ? 512 : 0), PIECES = XG + WG + (KIND == KIND_FP8 ? 2 : 0);
+  constexpr int STAGE = SCALES + (scaled(KIND) ? 512 : 0), PIECES = XG + WG + (scaled(KIND) ? 2 : 0);
   static_assert(D * NW * STAGE <= 160 * 1024 && 4 * MT * NT * 1024 <= D * NW * STAGE, "the rings fit into LDS, the join into the rings");
   static_assert(BM <= 64, "a lane loads one row's scale");
   __shared__ __attribute__((aligned(1024))) char smem[D * NW * STAGE];
@@ -506,8 +535,8 @@ __global__ __launch_bounds__(512, 2) void matmul_few_kernel(MatmulParams p) {
   for (int g = 0; g < XG; ++g) xoff[g] = (uint32_t)((source_row(8 * g + row0) - xfirst) * p.ldx);
 #pragma unroll
   for (int g = 0; g < WG; ++g) woff[g] = (uint32_t)(std::min(8 * g + row0, p.N - 1 - n0) * p.ldw);
-  const float* const xs = KIND == KIND_FP8 ? p.xs + source_row(lane) * p.xs_m : nullptr;       // (lanes >= BM: not used)
-  const float* const ws = KIND == KIND_FP8 ? p.ws + ((int64_t)e * ((p.N + 127) >> 7) + (n0 >> 7)) * p.nk : nullptr;
+  const float* const xs = scaled(KIND) ? p.xs + source_row(lane) * p.xs_m : nullptr;       // (lanes >= BM: not used)
+  const float* const ws = scaled(KIND) ? p.ws + ((int64_t)e * ((p.N + 127) >> 7) + (n0 >> 7)) * p.nk : nullptr;
   const int whole = p.Kb >> 7;
   char* const ring = smem + wave * (D * STAGE);
   auto fill = [&](int j, int st) {
@@ -522,7 +551,7 @@ __global__ __launch_bounds__(512, 2) void matmul_few_kernel(MatmulParams p) {
       const int c = ((lane & 7) ^ swz(8 * g + row0)) * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(wtile, (lds_ptr)(s + (2 * MT + g) * 1024), 16, woff[g] + (part && k0 + c >= p.Kb ? 0 : k0 + c), 0, 0, 0);
     }
-    if constexpr (KIND == KIND_FP8) {
+    if constexpr (scaled(KIND)) {
       __builtin_amdgcn_global_load_lds((gbl_ptr)(xs + kb * p.xs_b), (lds_ptr)(s + SCALES), 4, 0, 0);
       __builtin_amdgcn_global_load_lds((gbl_ptr)(ws + kb), (lds_ptr)(s + SCALES + 256), 4, 0, 0);
     }
@@ -554,9 +583,9 @@ __global__ __launch_bounds__(512, 2) void matmul_few_kernel(MatmulParams p) {
     for (int i = 0; i < MT; ++i) {
       const char* q = s + (16 * i + fr) * 128;
       x[i] = read_pair(q + (fg ^ (fr & 7)) * 16, q + ((fg + 4) ^ (fr & 7)) * 16);
-      sx[i] = KIND == KIND_FP8 ? reinterpret_cast<const float*>(s + SCALES)[16 * i + fr] : 0.f;
+      sx[i] = scaled(KIND) ? reinterpret_cast<const float*>(s + SCALES)[16 * i + fr] : 0.f;
     }
-    if constexpr (KIND == KIND_FP8) sw = reinterpret_cast<const float*>(s + SCALES)[64];
+    if constexpr (scaled(KIND)) sw = reinterpret_cast<const float*>(s + SCALES)[64];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the stage has been read: it may be filled again
     if (j + D < steps) fill(j + D, st);
     if (j * NW + wave == whole) {                          // what lies behind the row's end counts as zero
@@ -566,13 +595,21 @@ __global__ __launch_bounds__(512, 2) void matmul_few_kernel(MatmulParams p) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) x[i] = keep_pair(x[i], left);
     }
+    Wide ww[NT], xw;                                       // (KIND_FP8_WIDE)
+    if constexpr (KIND == KIND_FP8_WIDE) {
+#pragma unroll
+      for (int f = 0; f < NT; ++f) ww[f] = widen(w[f]);
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const float sc = sx[i] * sw;
+      if constexpr (KIND == KIND_FP8_WIDE) xw = widen(x[i]);
 #pragma unroll
       for (int f = 0; f < NT; ++f) {
-        if constexpr (KIND == KIND_FP8) {
-          const f32x4 part = mfma_step<KIND>(w[f], x[i], f32x4{0.f, 0.f, 0.f, 0.f});
+        if constexpr (scaled(KIND)) {
+          f32x4 part;
+          if constexpr (KIND == KIND_FP8) part = mfma_step<KIND>(w[f], x[i], f32x4{0.f, 0.f, 0.f, 0.f});
+          else part = mfma_wide(ww[f], xw);
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[i][f][q] = fmaf(part[q], sc, acc[i][f][q]);
         } else {
@@ -669,14 +706,19 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
     return cu * cu + l2 * l2 + once * once;
   };
   auto few = [&](int xg, int nt) {
-    const double block = p.nk * (xg + 2 * nt + (KIND == KIND_FP8 ? 2 : 0)) * 0.0112 + (GROUPED ? 2.8 : 0.3) + 0.1 * ((xg + 1) / 2 * nt);
+    const double block = p.nk * (xg + 2 * nt + (scaled(KIND) ? 2 : 0)) * 0.0112 + (GROUPED ? 2.8 : 0.3) + 0.1 * ((xg + 1) / 2 * nt);
     return time(8 * xg, 16 * nt, [&](double turns) { return turns * block; });
   };
   auto tiled = [&](int bm, int bn, double alone, double full, double ends) {
     return time(bm, bn, [&](double turns) { return turns == 1. ? p.nk * alone + ends : turns * (p.nk * full + ends); });
   };
-  const double t[] = {few(2, 1), few(2, 2), few(4, 2), few(6, 2), few(4, 4), few(6, 4), few(8, 4), tiled(64, 128, 0.34, 0.296, 0.4),
-                      tiled(128, 128, 0.47, 0.55, 1.5), tiled(128, 128, 0.53, 0.475, 1.3), tiled(128, 256, 0.8, 0.99, 3.8), tiled(256, 256, 1.22, 1.55, 10.)};
+  constexpr bool WIDE = KIND == KIND_FP8_WIDE;
+  const double t[] = {few(2, 1), few(2, 2), few(4, 2), few(6, 2), few(4, 4), few(6, 4), few(8, 4),
+                      WIDE ? tiled(64, 128, 0.6, 0.55, 0.4) : tiled(64, 128, 0.34, 0.296, 0.4),
+                      WIDE ? tiled(128, 128, 0.9, 1.0, 1.5) : tiled(128, 128, 0.47, 0.55, 1.5),
+                      WIDE ? tiled(128, 128, 1.0, 0.9, 1.3) : tiled(128, 128, 0.53, 0.475, 1.3),
+                      WIDE ? tiled(128, 256, 1.6, 1.9, 3.8) : tiled(128, 256, 0.8, 0.99, 3.8),
+                      WIDE ? HUGE_VAL : tiled(256, 256, 1.22, 1.55, 10.)};
   const auto least = std::min_element(std::begin(t), std::end(t));
   DIGA_CHECK_ARG(*least < HUGE_VAL, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)p.M, p.N);
   switch (least - t) {
@@ -691,7 +733,9 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
     case 8: launch_tile<KIND, 128, 128, 4, 2, 3, GROUPED>(p, s); break;
     case 9: launch_tile<KIND, 128, 128, 2, 2, 2, GROUPED>(p, s); break;
     case 10: launch_tile<KIND, 128, 256, 2, 4, 2, GROUPED>(p, s); break;
-    default: launch_tile<KIND, 256, 256, 2, 4, 2, GROUPED>(p, s); break;
+    default:                                               // (its wide form would take more than 256 registers)
+      if constexpr (!WIDE) launch_tile<KIND, 256, 256, 2, 4, 2, GROUPED>(p, s);
+      break;
   }
   DIGA_CHECK_LAUNCH(who);
   return DIGA_OK;
@@ -704,7 +748,6 @@ constexpr int MAX_ROW = 1 << 23;                           // bytes of an operan
 
 int check_product(const char* who, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* out, int out_type, int64_t ldo,
                   int64_t M, int N, int K, int size) {
-  DIGA_CHECK_ARG(size > 1 || out_type != DIGA_FP32, "%s: outputs of 8-bit products are bf16 or fp16 (the matrix pipe does not sum them to 32 bits)", who);
   DIGA_CHECK_ARG(M >= 0 && M <= MAX_M, "%s: M=%lld rows (0 .. 2^31 - 1024)", who, (long long)M);
   DIGA_CHECK_ARG(N >= 1 && N <= MAX_N && K >= 1 && K <= MAX_ROW / size, "%s: N=%d (1 .. 2^24), K=%d (1 .. 8 MiB of a row)", who, N, K);
   DIGA_CHECK_ARG(out_type == DIGA_BF16 || out_type == DIGA_FP16 || out_type == DIGA_FP32, "%s: unknown output type %d", who, out_type);
@@ -718,19 +761,36 @@ int check_product(const char* who, const void* x, int64_t ldx, const void* w, in
   return DIGA_OK;
 }
 
+int check_fp8_out(const char* who, int out_type) {
+  DIGA_CHECK_ARG(out_type != DIGA_FP32, "%s: outputs are bf16 or fp16 (the e4m3 matrix pipe does not sum them to 32 bits: %s_f32 does)", who, who);
+  return DIGA_OK;
+}
+
 }  // namespace
 
-extern "C" int diga_matmul_fp8(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
-                               const void* w, int64_t ldw, const float* w_scale, void* out, int out_type, int64_t ldo, int64_t M, int N,
-                               int K, void* stream) {
-  if (int rc = check_product("diga_matmul_fp8", x, ldx, w, ldw, out, out_type, ldo, M, N, K, 1)) return rc;
+template <int KIND>
+static int dense_fp8(const char* who, const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
+                     const void* w, int64_t ldw, const float* w_scale, void* out, int out_type, int64_t ldo, int64_t M, int N, int K, void* stream) {
+  if (int rc = check_product(who, x, ldx, w, ldw, out, out_type, ldo, M, N, K, 1)) return rc;
   if (M == 0) return DIGA_OK;
-  DIGA_CHECK_ARG(x_scale && w_scale, "diga_matmul_fp8: null pointer");
+  DIGA_CHECK_ARG(x_scale && w_scale, "%s: null pointer", who);
   MatmulParams p{};
   p.x = (const char*)x, p.w = (const char*)w, p.xs = x_scale, p.ws = w_scale, p.out = out;
   p.ldx = ldx, p.ldw = ldw, p.xs_m = x_scale_stride_m, p.xs_b = x_scale_stride_b, p.ldo = ldo;
   p.M = M, p.xrows = M, p.N = N, p.Kb = K, p.nk = cdiv(K, 128), p.E = 1, p.out_type = out_type;
-  return launch<KIND_FP8, false>("diga_matmul_fp8", p, static_cast<hipStream_t>(stream));
+  return launch<KIND, false>(who, p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int diga_matmul_fp8(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
+                               const void* w, int64_t ldw, const float* w_scale, void* out, int out_type, int64_t ldo, int64_t M, int N,
+                               int K, void* stream) {
+  if (int rc = check_fp8_out("diga_matmul_fp8", out_type)) return rc;
+  return dense_fp8<KIND_FP8>("diga_matmul_fp8", x, ldx, x_scale, x_scale_stride_m, x_scale_stride_b, w, ldw, w_scale, out, out_type, ldo, M, N, K, stream);
+}
+
+extern "C" int diga_matmul_fp8_f32(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
+                                   const void* w, int64_t ldw, const float* w_scale, float* out, int64_t ldo, int64_t M, int N, int K, void* stream) {
+  return dense_fp8<KIND_FP8_WIDE>("diga_matmul_fp8_f32", x, ldx, x_scale, x_scale_stride_m, x_scale_stride_b, w, ldw, w_scale, out, DIGA_FP32, ldo, M, N, K, stream);
 }
 
 static int check_groups(const char* who, const int32_t* offsets, int groups, const int32_t* rows, int64_t x_rows, int64_t T, int64_t ldx_bytes, int64_t row_bytes, int64_t ldw, int64_t w_stride, int N) {
@@ -744,11 +804,10 @@ static int check_groups(const char* who, const int32_t* offsets, int groups, con
   return DIGA_OK;
 }
 
-extern "C" int diga_grouped_matmul_fp8(const void* x, int64_t ldx, int64_t x_rows, const float* x_scale, int64_t x_scale_stride_m,
-                                       int64_t x_scale_stride_b, const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride,
-                                       const float* w_scale, const int32_t* offsets, int groups, void* out, int out_type, int64_t ldo,
-                                       int64_t T, int N, int K, void* stream) {
-  const char* who = "diga_grouped_matmul_fp8";
+template <int KIND>
+static int grouped_fp8(const char* who, const void* x, int64_t ldx, int64_t x_rows, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
+                       const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride, const float* w_scale, const int32_t* offsets, int groups,
+                       void* out, int out_type, int64_t ldo, int64_t T, int N, int K, void* stream) {
   if (int rc = check_product(who, x, ldx, w, ldw, out, out_type, ldo, T, N, K, 1)) return rc;
   if (int rc = check_groups(who, offsets, groups, rows, x_rows, T, ldx, (K + 15) / 16 * 16, ldw, w_stride, N)) return rc;
   DIGA_CHECK_ARG(w_stride % 16 == 0, "%s: weight matrices must start at multiples of 16 bytes", who);
@@ -758,7 +817,24 @@ extern "C" int diga_grouped_matmul_fp8(const void* x, int64_t ldx, int64_t x_row
   p.x = (const char*)x, p.w = (const char*)w, p.xs = x_scale, p.ws = w_scale, p.rows = rows, p.offsets = offsets, p.out = out;
   p.ldx = ldx, p.ldw = ldw, p.wstride = w_stride, p.xs_m = x_scale_stride_m, p.xs_b = x_scale_stride_b, p.ldo = ldo;
   p.M = T, p.xrows = x_rows, p.N = N, p.Kb = K, p.nk = cdiv(K, 128), p.E = groups, p.out_type = out_type;
-  return launch<KIND_FP8, true>(who, p, static_cast<hipStream_t>(stream));
+  return launch<KIND, true>(who, p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int diga_grouped_matmul_fp8(const void* x, int64_t ldx, int64_t x_rows, const float* x_scale, int64_t x_scale_stride_m,
+                                       int64_t x_scale_stride_b, const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride,
+                                       const float* w_scale, const int32_t* offsets, int groups, void* out, int out_type, int64_t ldo,
+                                       int64_t T, int N, int K, void* stream) {
+  if (int rc = check_fp8_out("diga_grouped_matmul_fp8", out_type)) return rc;
+  return grouped_fp8<KIND_FP8>("diga_grouped_matmul_fp8", x, ldx, x_rows, x_scale, x_scale_stride_m, x_scale_stride_b, rows, w, ldw, w_stride, w_scale,
+                               offsets, groups, out, out_type, ldo, T, N, K, stream);
+}
+
+extern "C" int diga_grouped_matmul_fp8_f32(const void* x, int64_t ldx, int64_t x_rows, const float* x_scale, int64_t x_scale_stride_m,
+                                           int64_t x_scale_stride_b, const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride,
+                                           const float* w_scale, const int32_t* offsets, int groups, float* out, int64_t ldo, int64_t T, int N,
+                                           int K, void* stream) {
+  return grouped_fp8<KIND_FP8_WIDE>("diga_grouped_matmul_fp8_f32", x, ldx, x_rows, x_scale, x_scale_stride_m, x_scale_stride_b, rows, w, ldw, w_stride, w_scale,
+                                    offsets, groups, out, DIGA_FP32, ldo, T, N, K, stream);
 }
 
 extern "C" int diga_grouped_matmul(const void* x, int64_t ldx, int64_t x_rows, int type, const int32_t* rows, const void* w, int64_t ldw,

@@ -67,6 +67,7 @@ class _Entry:
 
 _rms_norm, _silu_mul, _quantize = _Entry("diga_rms_norm_fp8"), _Entry("diga_silu_mul_fp8"), _Entry("diga_quantize_fp8")
 _matmul, _grouped_fp8, _grouped = _Entry("diga_matmul_fp8"), _Entry("diga_grouped_matmul_fp8"), _Entry("diga_grouped_matmul")
+_matmul_f32, _grouped_fp8_f32 = _Entry("diga_matmul_fp8_f32"), _Entry("diga_grouped_matmul_fp8_f32")
 
 
 def _device(who, *tensors):
@@ -114,9 +115,9 @@ def _operand(who, name, t, rows, cols, ld, piece):
     return ld if rows > 1 else whole
 
 
-def _check_out(who, out, m, n, dtype, dtypes=_TYPES):
-    if dtype not in dtypes:
-        raise DigaError(f"{who}: outputs are {', '.join(str(d) for d in dtypes)}, not {dtype}")
+def _check_out(who, out, m, n, dtype):
+    if dtype not in _TYPES:
+        raise DigaError(f"{who}: outputs are {', '.join(str(d) for d in _TYPES)}, not {dtype}")
     if out is not None and (out.dtype is not dtype or out.shape != (m, n) or (n > 1 and out.stride(1) != 1)):
         raise DigaError(f"{who}: out must be {dtype} ({m}, {n}) with adjacent columns, got {out.dtype} {tuple(out.shape)} with strides {out.stride()}")
 
@@ -217,10 +218,20 @@ def _check_scales(who, xs, ws, m, k, lead):
     return xs.stride()
 
 
+def _check_wide(who, out_dtype, x):
+    if out_dtype is torch.float32 and not x.is_cuda:
+        raise DigaError(f"{who}: float32 outputs are summed from 16-bit operands on the GPU: there is no CPU fallback")
+
+
+def _fp8_entry(out_dtype, halves, f32):
+    """The entry point for outputs of out_dtype, and its argument that says which."""
+    return (f32, ()) if out_dtype is torch.float32 else (halves, (_HALVES[out_dtype],))
+
+
 def matmul_fp8(xq, xs, wq, ws, out_dtype=torch.bfloat16, out=None):
     """x @ w.T of 8-bit rows and weights: xq e4m3 [M, K] with xs fp32 [M, ceil(K / 128)], wq e4m3 [N, K] with ws fp32
-    [ceil(N / 128), ceil(K / 128)] -> [M, N] of out_dtype (bf16 / fp16), fp32 sums over the blocks, rounded once.  Rows of xq and wq start
-    at multiples of 16 bytes."""
+    [ceil(N / 128), ceil(K / 128)] -> [M, N] of out_dtype (bf16 / fp16 / fp32), fp32 sums over the blocks, rounded once.  Rows of xq and wq start
+    at multiples of 16 bytes.  For fp32 the products are summed in 32 bits too, at half the matrix rate."""
     done = _calls.matmul(xq, xs, wq, ws, out_dtype, out)
     if done is not None:
         return done
@@ -231,12 +242,13 @@ def matmul_fp8(xq, xs, wq, ws, out_dtype=torch.bfloat16, out=None):
         raise DigaError(f"{who}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)} do not fit")
     sm, sb = _check_scales(who, xs, ws, m, k, (-(-n // BLOCK),))
     ldx, ldw = _operand(who, "xq", xq, m, k, ldx, 16), _operand(who, "wq", wq, n, k, ldw, 16)
-    _check_out(who, out, m, n, out_dtype, _HALVES)
+    _check_out(who, out, m, n, out_dtype)
+    _check_wide(who, out_dtype, xq)
     index = _device(who, xq, xs, wq, ws, out)
     if out is None:
         out = _empty((m, n), dtype=out_dtype, device=xq.device)
-    _matmul(index, xq.data_ptr(), ldx, xs.data_ptr(), sm, sb, wq.data_ptr(), ldw, ws.data_ptr(), out.data_ptr(), _HALVES[out_dtype],
-            out.stride(0), m, n, k)
+    entry, kind = _fp8_entry(out_dtype, _matmul, _matmul_f32)
+    entry(index, xq.data_ptr(), ldx, xs.data_ptr(), sm, sb, wq.data_ptr(), ldw, ws.data_ptr(), out.data_ptr(), *kind, out.stride(0), m, n, k)
     return out
 
 
@@ -265,12 +277,14 @@ def grouped_matmul_fp8(xq, xs, wq, ws, offsets, rows=None, out_dtype=torch.bfloa
     who = "grouped_matmul_fp8"
     xr, k, e, n, t, we, ldx, ldw = _groups(who, xq, wq, offsets, rows, _E4M3, 16)
     sm, sb = _check_scales(who, xs, ws, xr, k, (e, -(-n // BLOCK)))
-    _check_out(who, out, t, n, out_dtype, _HALVES)
+    _check_out(who, out, t, n, out_dtype)
+    _check_wide(who, out_dtype, xq)
     index = _device(who, xq, xs, wq, ws, offsets, rows, out)
     if out is None:
         out = _empty((t, n), dtype=out_dtype, device=xq.device)
-    _grouped_fp8(index, xq.data_ptr(), ldx, xr, xs.data_ptr(), sm, sb, rows.data_ptr() if rows is not None else None, wq.data_ptr(), ldw,
-                 we, ws.data_ptr(), offsets.data_ptr(), e, out.data_ptr(), _HALVES[out_dtype], out.stride(0), t, n, k)
+    entry, kind = _fp8_entry(out_dtype, _grouped_fp8, _grouped_fp8_f32)
+    entry(index, xq.data_ptr(), ldx, xr, xs.data_ptr(), sm, sb, rows.data_ptr() if rows is not None else None, wq.data_ptr(), ldw,
+          we, ws.data_ptr(), offsets.data_ptr(), e, out.data_ptr(), *kind, out.stride(0), t, n, k)
     return out
 
 

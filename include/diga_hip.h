@@ -463,6 +463,14 @@ int diga_grouped_matmul_fp8(const void* x, int64_t ldx, int64_t x_rows, const fl
                             int64_t x_scale_stride_b, const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride,
                             const float* w_scale, const int32_t* offsets, int groups, void* out, int out_type,
                             int64_t ldo, int64_t T, int N, int K, void* stream);
+/* Both with fp32 outputs: the operands are made bf16 in registers (exact) and their products summed in fp32, at half the matrix rate. */
+int diga_matmul_fp8_f32(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m, int64_t x_scale_stride_b,
+                        const void* w, int64_t ldw, const float* w_scale, float* out, int64_t ldo, int64_t M, int N, int K,
+                        void* stream);
+int diga_grouped_matmul_fp8_f32(const void* x, int64_t ldx, int64_t x_rows, const float* x_scale, int64_t x_scale_stride_m,
+                                int64_t x_scale_stride_b, const int32_t* rows, const void* w, int64_t ldw, int64_t w_stride,
+                                const float* w_scale, const int32_t* offsets, int groups, float* out, int64_t ldo, int64_t T,
+                                int N, int K, void* stream);
 /* The same on bf16 / fp16 operands (`type`), no scales: out = x . w[e]^T, fp32 sums, out_type any. */
 int diga_grouped_matmul(const void* x, int64_t ldx, int64_t x_rows, int type, const int32_t* rows, const void* w,
                         int64_t ldw, int64_t w_stride, const int32_t* offsets, int groups, void* out, int out_type,
