@@ -86,6 +86,12 @@ def _device(who, *tensors):
     return index
 
 
+def _counts(who, what, n):
+    """The entry points take columns, weight rows and groups as 32-bit integers, which ctypes would cut off without a word."""
+    if n >= 1 << 31:
+        raise DigaError(f"{who}: {n} {what} are more than 2^31 - 1")
+
+
 def _rows(who, name, t, dtypes):
     """A matrix whose columns are adjacent, of one of `dtypes` -> (rows, columns, row stride)."""
     if t.dim() == 2:
@@ -93,6 +99,7 @@ def _rows(who, name, t, dtypes):
         ld, step = t.stride()
         if n and (step == 1 or n == 1):
             if t.dtype in dtypes:
+                _counts(who, f"columns of {name}", n)
                 return m, n, ld
             raise DigaError(f"{who}: {name} is {t.dtype}, not one of {', '.join(str(d) for d in dtypes)}")
     raise DigaError(f"{who}: {name} must be a matrix with adjacent columns, got {tuple(t.shape)} with strides {t.stride()}")
@@ -240,6 +247,7 @@ def matmul_fp8(xq, xs, wq, ws, out_dtype=torch.bfloat16, out=None):
     n, kw, ldw = _rows(who, "wq", wq, _E4M3)
     if k != kw or n == 0:
         raise DigaError(f"{who}: xq {tuple(xq.shape)} and wq {tuple(wq.shape)} do not fit")
+    _counts(who, "rows of wq", n)
     sm, sb = _check_scales(who, xs, ws, m, k, (-(-n // BLOCK),))
     ldx, ldw = _operand(who, "xq", xq, m, k, ldx, 16), _operand(who, "wq", wq, n, k, ldw, 16)
     _check_out(who, out, m, n, out_dtype)
@@ -257,6 +265,8 @@ def _groups(who, x, w, offsets, rows, dtypes, piece):
     if w.dim() != 3 or w.dtype is not x.dtype or w.shape[2] != k or 0 in w.shape or (k > 1 and w.stride(2) != 1):
         raise DigaError(f"{who}: weights must be {x.dtype} (experts, N, {k}) with adjacent columns, got {w.dtype} {tuple(w.shape)} with strides {w.stride()}")
     e, n, _ = w.shape
+    _counts(who, "weight rows", n)
+    _counts(who, "weight matrices", e)
     _plain(who, "offsets", offsets, torch.int32, (e + 1,))
     t = xr
     if rows is not None:
