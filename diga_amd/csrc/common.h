@@ -60,4 +60,16 @@ __device__ __forceinline__ u32x4 pack_bf16x8(const float* f) {
   return v;
 }
 
+// Whether two sets of rows (`wide` bytes each, `ld` bytes apart) share memory.  Rows of one stride may lie side by side in a wider matrix;
+// where strides differ, ranges that meet count as shared.
+static inline bool rows_meet(const void* a, int64_t a_rows, int64_t a_ld, int64_t a_wide, const void* b, int64_t b_rows, int64_t b_ld, int64_t b_wide) {
+  const int64_t a0 = (int64_t)(uintptr_t)a, b0 = (int64_t)(uintptr_t)b;
+  if (a0 + (a_rows - 1) * a_ld + a_wide <= b0 || b0 + (b_rows - 1) * b_ld + b_wide <= a0) return false;
+  if (a_rows == 1) a_ld = b_ld;
+  if (b_rows == 1) b_ld = a_ld;
+  if ((a_rows == 1 && b_rows == 1) || a_ld != b_ld || a_wide > a_ld || b_wide > a_ld) return true;
+  const int64_t d = ((b0 - a0) % a_ld + a_ld) % a_ld;
+  return d < a_wide || d + b_wide > a_ld;
+}
+
 static inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }

@@ -721,6 +721,11 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
                       WIDE ? HUGE_VAL : tiled(256, 256, 1.22, 1.55, 10.)};
   const auto least = std::min_element(std::begin(t), std::end(t));
   DIGA_CHECK_ARG(*least < HUGE_VAL, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)p.M, p.N);
+  const int64_t size = p.out_type == DIGA_FP32 ? 4 : 2;
+  DIGA_CHECK_ARG(!rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.x, p.rows ? p.xrows : p.M, p.ldx, p.Kb), "%s: the output lies on the left rows", who);
+  DIGA_CHECK_ARG(!(p.E == 1 ? rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.w, p.N, p.ldw, p.Kb)
+                            : rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.w, p.E, p.wstride, (p.N - 1) * p.ldw + p.Kb)),
+                 "%s: the output lies on the weights", who);
   switch (least - t) {
     case 0: launch_few<KIND, 2, 1, 2, GROUPED>(p, s); break;
     case 1: launch_few<KIND, 2, 2, 2, GROUPED>(p, s); break;

@@ -238,12 +238,19 @@ extern "C" int diga_rms_norm_fp8(const void* x, int64_t ldx, const void* residua
   DIGA_CHECK_ARG(eps >= 0.f, "diga_rms_norm_fp8: eps must not be negative");
   if (M == 0) return DIGA_OK;
   DIGA_CHECK_ARG(weight, "diga_rms_norm_fp8: null pointer");
+  const int64_t size = type == DIGA_FP32 ? 4 : 2, wsize = weight_type == DIGA_FP32 ? 4 : 2;
+  if (residual) {                                          // x or the residual itself may take the sum, nothing that lies across them
+    const bool on_x = residual_out == x && (M == 1 || ldh == ldx), on_res = residual_out == residual && (M == 1 || ldh == ldr);
+    DIGA_CHECK_ARG((on_x || !rows_meet(residual_out, M, ldh * size, N * size, x, M, ldx * size, N * size)) &&
+                       (on_res || !rows_meet(residual_out, M, ldh * size, N * size, residual, M, ldr * size, N * size)) &&
+                       !rows_meet(residual_out, M, ldh * size, N * size, weight, 1, 0, N * wsize),
+                   "diga_rms_norm_fp8: residual_out lies across x, the residual or the weight");
+  }
   RowQuantParams p{};
   p.x = x, p.res = residual, p.weight = weight, p.q = static_cast<uint8_t*>(q), p.scale = scale, p.h = residual_out;
   p.M = M, p.N = N, p.nb = cdiv(N, 128), p.ldx = ldx, p.ldr = ldr, p.ldq = ldq, p.ldh = ldh, p.ssm = scale_stride_m, p.ssb = scale_stride_b;
   p.wtype = weight_type, p.eps = eps;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t size = type == DIGA_FP32 ? 4 : 2;
   for (int64_t done = 0; done < M; done += RMS_ROWS) {     // a launch has fewer than 2^32 threads, up to 1024 of them a row
     p.M = std::min(M - done, RMS_ROWS);
     if (type == DIGA_BF16) launch_rms<__bf16>(p, s);

@@ -12,7 +12,8 @@ scale per 128 x 128 block.  One gated block of an encoder, dense or by expert:
 
 Everything is enqueued on the current stream of the tensors' device, allocates through torch and can be captured into a graph.
 Scales of rows come back as a [rows, blocks] view whose rows lie side by side in memory (stride 1), the layout the products read
-fastest; any strides are accepted.  There is no CPU path and no backward pass: tensors are taken detached.
+fastest; any strides are accepted.  A call that would write a result over its own operands is refused, but for a norm's residual_out on x
+or the residual.  There is no CPU path and no backward pass: tensors are taken detached.
 """
 from __future__ import annotations
 

@@ -435,7 +435,7 @@ int diga_nhwc_f32_to_nchw_f32(const float* in, float* out, int B, int HW, int C,
  * ------------------------------------------------------------------------------------------ */
 /* h = x (+ residual); y = h * weight / sqrt(mean(h^2) + eps), all in fp32; per row and block of 128 columns
  * scale = max(max|y|, 2^-100) / 448, q = e4m3(y / scale) (nearest even).  With a residual, h is also written to residual_out,
- * rounded to `type`; residual_out may be x or residual themselves (same stride).  A NaN of y stays at its place; the row's scales
+ * rounded to `type`; residual_out may be x or residual themselves (same stride), and is refused where it lies across them or the weight otherwise.  A NaN of y stays at its place; the row's scales
  * are those of its numbers.  x, residual, residual_out: `type`, weight [N]: weight_type.  N <= DIGA_RMS_NORM_MAX_N. */
 #define DIGA_RMS_NORM_MAX_N 65536
 int diga_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, int type, const void* weight,
@@ -451,7 +451,7 @@ int diga_quantize_fp8(const void* x, int64_t ldx, int type, int64_t M, int N, vo
  * out_type (DIGA_BF16 or DIGA_FP16: the matrix pipe adds 8 e4m3 products with 13 bits below the largest, 2e-5 .. 5e-5 of a result, which
  * would not make a 32-bit one).  x: e4m3 [M][K]; w: e4m3 [N][K]; w_scale: fp32 [ceil(N/128)][ceil(K/128)]; out [M][N].
  * x and w rows start at multiples of 16 bytes (base and stride); a row's bytes up to K rounded up to 16 must be readable, what they
- * hold does not matter.  No scratch memory. */
+ * hold does not matter.  out may not lie on x or w.  No scratch memory. */
 int diga_matmul_fp8(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m,
                     int64_t x_scale_stride_b, const void* w, int64_t ldw, const float* w_scale, void* out, int out_type,
                     int64_t ldo, int64_t M, int N, int K, void* stream);
