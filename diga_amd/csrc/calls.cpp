@@ -6,6 +6,7 @@
 // nothing, and the Python function goes on with its own checks: it alone says what is wrong, and takes the rarer layouts.  A launch
 // that fails raises here: a second one of a norm in place would add the residual twice.
 #include <Python.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -41,11 +42,14 @@ int gpu_of(PyObject* obj) {
   const int index = t.get_device();
   return index == c10::hip::current_device() ? index : -1;
 }
-// obj as a plain tensor on GPU `index` that no gradient is asked of; NULL otherwise
+// whether forward-mode differentiation would take t's tangent through the call
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode(); }
+// obj as a plain tensor on GPU `index` that no derivative is asked of; NULL otherwise
 const at::Tensor* plain(PyObject* obj, int index) {
   if (!THPVariable_CheckExact(obj)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(obj);
-  return t.is_cuda() && t.get_device() == index && t.layout() == at::kStrided && !(t.requires_grad() && c10::GradMode::is_enabled()) && !t.is_neg() ? &t : nullptr;
+  if (!t.is_cuda() || t.get_device() != index || t.layout() != at::kStrided || t.is_neg()) return nullptr;
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || has_tangent(t) ? nullptr : &t;
 }
 // a matrix with adjacent columns
 bool matrix(const at::Tensor& t, ScalarType type) { return t.dim() == 2 && t.scalar_type() == type && t.size(1) > 0 && t.stride(1) == 1; }

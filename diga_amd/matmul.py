@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from ._lib import DigaError, check, load
 
@@ -41,6 +42,7 @@ _HALVES = {torch.bfloat16: 0, torch.float16: 1}
 _E4M3 = {E4M3: 0}
 _stream_of = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_fwd_grad_enabled = torch._C._is_fwd_grad_enabled
 _empty, _strided = torch.empty, torch.empty_strided
 
 
@@ -84,6 +86,8 @@ def _device(who, *tensors):
                 raise DigaError(f"{who}: a tensor's values are held negated: pass its resolve_neg()")
             if t.requires_grad and torch.is_grad_enabled():
                 raise DigaError(f"{who} has no backward pass: call it under torch.no_grad() or on detached tensors")
+            if _fwd_grad_enabled() and unpack_dual(t).tangent is not None:
+                raise DigaError(f"{who} has no derivative: a tensor carries a tangent, which would be dropped: pass it without")
     return index
 
 

@@ -1,6 +1,7 @@
 """-m gpu: calls of diga_amd/matmul.py at the edge of what it takes."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import matmul_ref as R
 from diga_amd import matmul as M
@@ -55,3 +56,30 @@ def test_one_output_row_between_the_rows_of_its_operands():
     R.check_product(want, R.rows_of(xq, xs), R.weights_of(wq, ws), True)
     with pytest.raises(DigaError, match="the output lies on the weights"):
         M.matmul_fp8(xq, xs, rows[:, :256].view(E4M3), ws, out=rows[5:6, 240:304].view(BF16))
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_tensors_with_a_tangent_are_refused(strided):
+    """Forward-mode differentiation, on the ordinary call and on the one that goes by the Python checks."""
+    g = gen(3)
+    x, w, r = rand(g, 6, 256).bfloat16(), rand(g, 128).bfloat16(), rand(g, 6, 128).bfloat16()
+    x = x[:, :128] if strided else x[:, :128].contiguous()
+    q, s = M.quantize_fp8(x)
+    wq, ws = M.quantize_weight_fp8(rand(g, 2, 40, 128))
+    off = sizes_to_offsets([2, 4])
+    w16 = rand(g, 2, 40, 128).bfloat16()
+    eps = 1 if strided else 1e-6
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: M.rms_norm_fp8(dual(x), w, None, eps), lambda: M.rms_norm_fp8(x, dual(w), None, eps), lambda: M.rms_norm_fp8(x, w, dual(r), eps),
+                     lambda: M.silu_mul_fp8(dual(x)), lambda: M.quantize_fp8(dual(x)), lambda: M.matmul_fp8(q, dual(s), wq[0], ws[0]),
+                     lambda: M.matmul_fp8(q, s, wq[0], dual(ws[0]), torch.float32), lambda: M.grouped_matmul(dual(x), w16, off),
+                     lambda: M.grouped_matmul(x, dual(w16), off), lambda: M.grouped_matmul_fp8(q, dual(s), wq, ws, off)):
+            with pytest.raises(DigaError, match="tangent"):
+                call()
+        with torch.no_grad(), pytest.raises(DigaError, match="tangent"):    # (no_grad leaves forward mode on)
+            M.quantize_fp8(dual(x))
+        p = dual(x)
+        assert torch.equal(M.quantize_fp8(fwd.unpack_dual(p).primal)[0].float(), q.float())
+        with fwd._set_fwd_grad_enabled(False):
+            assert torch.equal(M.quantize_fp8(p)[0].float(), q.float())
