@@ -70,6 +70,11 @@ struct Rows {
 
 void* stream(int index) { return c10::hip::getCurrentHIPStream(index).stream(); }
 
+// t was written in place: a later backward that saved it has to notice (inference tensors count no versions)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* none() { Py_RETURN_NONE; }
 
 // an entry point returned rc < 0: arguments it refuses are left to Python
@@ -108,7 +113,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                             r ? h.mutable_data_ptr() : nullptr, r ? h.stride(0) : 0, stream(index));
   if (rc < 0) return failed("diga_rms_norm_fp8", rc);
   PyObject* hobj = Py_None;
-  if (given) hobj = a[4];
+  if (given) written(*given), hobj = a[4];
   if (!r || given) Py_INCREF(hobj);
   else hobj = THPVariable_Wrap(std::move(h));
   return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(out.q)), THPVariable_Wrap(std::move(out.scale)), hobj);
@@ -151,6 +156,7 @@ bool output(PyObject* given, int index, int64_t m, int64_t n, ScalarType type, c
 }
 PyObject* returned(PyObject* given, at::Tensor&& out) {
   if (given == Py_None) return THPVariable_Wrap(std::move(out));
+  written(out);
   Py_INCREF(given);
   return given;
 }

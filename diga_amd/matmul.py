@@ -21,6 +21,7 @@ import ctypes
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
+from torch.autograd.graph import increment_version as _written      # a tensor written in place: a backward that saved it has to notice
 
 from ._lib import DigaError, check, load
 
@@ -175,6 +176,8 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, residual_out=None):
     q, ldq, s = _empty_rows(m, n, x.device)
     _rms_norm(index, x.data_ptr(), ldx, r, ldr, _TYPES[dtype], weight.data_ptr(), _TYPES[weight.dtype], eps, m, n, q.data_ptr(), ldq,
               s.data_ptr(), 1, m, h, ldh)
+    if h is not None:
+        _written(residual_out)
     return q, s, residual_out
 
 
@@ -262,6 +265,7 @@ def matmul_fp8(xq, xs, wq, ws, out_dtype=torch.bfloat16, out=None):
         out = _empty((m, n), dtype=out_dtype, device=xq.device)
     entry, kind = _fp8_entry(out_dtype, _matmul, _matmul_f32)
     entry(index, xq.data_ptr(), ldx, xs.data_ptr(), sm, sb, wq.data_ptr(), ldw, ws.data_ptr(), out.data_ptr(), *kind, out.stride(0), m, n, k)
+    _written(out)
     return out
 
 
@@ -300,6 +304,7 @@ def grouped_matmul_fp8(xq, xs, wq, ws, offsets, rows=None, out_dtype=torch.bfloa
     entry, kind = _fp8_entry(out_dtype, _grouped_fp8, _grouped_fp8_f32)
     entry(index, xq.data_ptr(), ldx, xr, xs.data_ptr(), sm, sb, rows.data_ptr() if rows is not None else None, wq.data_ptr(), ldw,
           we, ws.data_ptr(), offsets.data_ptr(), e, out.data_ptr(), *kind, out.stride(0), t, n, k)
+    _written(out)
     return out
 
 
@@ -317,4 +322,5 @@ def grouped_matmul(x, w, offsets, rows=None, out_dtype=None, out=None):
         out = _empty((t, n), dtype=out_dtype, device=x.device)
     _grouped(index, x.data_ptr(), ldx, xr, _HALVES[x.dtype], rows.data_ptr() if rows is not None else None, w.data_ptr(), ldw, we,
              offsets.data_ptr(), e, out.data_ptr(), _TYPES[out_dtype], out.stride(0), t, n, k)
+    _written(out)
     return out

@@ -6,7 +6,7 @@ import torch.autograd.forward_ad as fwd
 import matmul_ref as R
 from diga_amd import matmul as M
 from diga_amd._lib import DigaError
-from test_gpu_matmul import BF16, DEV, E4M3, gen, held, held_weights, rand, sizes_to_offsets
+from test_gpu_matmul import BF16, DEV, E4M3, NothingShort, gen, held, held_weights, rand, sizes_to_offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,29 @@ def test_tensors_with_a_tangent_are_refused(strided):
         assert torch.equal(M.quantize_fp8(fwd.unpack_dual(p).primal)[0].float(), q.float())
         with fwd._set_fwd_grad_enabled(False):
             assert torch.equal(M.quantize_fp8(p)[0].float(), q.float())
+
+
+@pytest.mark.parametrize("long_way", [False, True])
+def test_a_backward_notices_what_was_written_in_place(monkeypatch, long_way):
+    if long_way:
+        monkeypatch.setattr(M, "_calls", NothingShort())
+    g = gen(4)
+    x, r, w = rand(g, 6, 128).bfloat16(), rand(g, 6, 128).bfloat16(), torch.ones(128, dtype=BF16, device=DEV)
+    q, s = M.quantize_fp8(x)
+    wq, ws = M.quantize_weight_fp8(rand(g, 2, 128, 128))
+    w16, off = rand(g, 2, 128, 128).bfloat16(), sizes_to_offsets([2, 4])
+    fp32 = torch.float32
+    for dtype, write in [(BF16, lambda t: M.rms_norm_fp8(x, w, r, 1e-6, t)), (BF16, lambda t: M.rms_norm_fp8(t, w, r, 1e-6, t)), (BF16, lambda t: M.matmul_fp8(q, s, wq[0], ws[0], out=t)),
+                         (fp32, lambda t: M.matmul_fp8(q, s, wq[0], ws[0], fp32, t)), (BF16, lambda t: M.grouped_matmul_fp8(q, s, wq, ws, off, out=t)),
+                         (fp32, lambda t: M.grouped_matmul_fp8(q, s, wq, ws, off, None, fp32, t)), (fp32, lambda t: M.grouped_matmul(x, w16, off, None, fp32, t))]:
+        saved, leaf = rand(g, 6, 128).to(dtype), torch.ones(6, 128, dtype=dtype, device=DEV, requires_grad=True)
+        loss = (leaf * saved).sum()           # the backward needs `saved` as it is now
+        write(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        kept = torch.empty(6, 128, dtype=BF16, device=DEV)
+        M.matmul_fp8(q, s, wq[0], ws[0], out=kept)
+    again = torch.empty_like(kept)
+    M.matmul_fp8(q, s, wq[0], ws[0], out=kept)                          # outside as well: nothing can have saved it
+    assert torch.equal(kept, M.matmul_fp8(q, s, wq[0], ws[0], out=again))
