@@ -690,12 +690,17 @@ void launch_few(MatmulParams p, hipStream_t s) {
 //             128 x 128, 4 waves, 2 stages, two on a CU: 0.53, 0.475, 1.3 (8385 x 2048 x 2048: 45.0; others 49.3, 54.7, 61.2)
 //             128 x 256, 8 waves, 2 stages, one on a CU: 0.8, 0.99, 3.8 (5482 x 1000 x 2048 bf16 in 16 groups: 32.2; 37.9, 42.5, 40.9, 48.7)
 //             256 x 256, 8 waves, 2 stages, one on a CU: 1.22, 1.55, 10 (8192^3: 440; others 622, 592, 503, 524)
+//   fp32 outputs of 8-bit products: half the matrix rate, and the widening: few + 0.012 per K step and accumulator; tiled in the order above 0.7,
+//             0.53, 0.4; 1.02, 1.05, 1.5; 1.0, 0.87, 1.7; 1.6, 1.8, 5 (picks within 1.01 of the best of 11 over 28 sizes, dense and grouped: 517 x 1001 x
+//             2064: 48 x 64 9.7, 64 x 64 10.8, 64 x 128 15.4; 256 x 4096 x 4096: 64 x 64 15.2, 64 x 128 23.7; 8192^3: 128 x 128 of 4 waves 906, 128 x 256
+//             912, 64 x 128 1099; the wide 256 x 256 tile would take more than 256 registers)
 // (e4m3, M x N x K; a step of 16-bit operands is half the K and the same bytes and MFMA clocks.)
 // A launch has fewer than 2^32 threads: tiles that would need 2^23 blocks of 512 are left out.
 constexpr int64_t MAX_BLOCKS = ((int64_t)1 << 23) - 1;
 
 template <int KIND, bool GROUPED>
 int launch(const char* who, const MatmulParams& p, hipStream_t s) {
+  constexpr bool WIDE = KIND == KIND_FP8_WIDE;
   const double groups = GROUPED ? (double)std::min<int64_t>(p.E, p.M) : 1., avg = (double)p.M / groups;
   const double once = ((double)p.xrows + groups * p.N) * p.Kb / 4.9e6;
   auto time = [&](int bm, int bn, auto work) {
@@ -706,18 +711,17 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
     return cu * cu + l2 * l2 + once * once;
   };
   auto few = [&](int xg, int nt) {
-    const double block = p.nk * (xg + 2 * nt + (scaled(KIND) ? 2 : 0)) * 0.0112 + (GROUPED ? 2.8 : 0.3) + 0.1 * ((xg + 1) / 2 * nt);
+    const double block = p.nk * (xg + 2 * nt + (scaled(KIND) ? 2 : 0)) * 0.0112 + (GROUPED ? 2.8 : 0.3) + (0.1 + (WIDE ? 0.012 * p.nk : 0.)) * ((xg + 1) / 2 * nt);
     return time(8 * xg, 16 * nt, [&](double turns) { return turns * block; });
   };
   auto tiled = [&](int bm, int bn, double alone, double full, double ends) {
     return time(bm, bn, [&](double turns) { return turns == 1. ? p.nk * alone + ends : turns * (p.nk * full + ends); });
   };
-  constexpr bool WIDE = KIND == KIND_FP8_WIDE;
   const double t[] = {few(2, 1), few(2, 2), few(4, 2), few(6, 2), few(4, 4), few(6, 4), few(8, 4),
-                      WIDE ? tiled(64, 128, 0.6, 0.55, 0.4) : tiled(64, 128, 0.34, 0.296, 0.4),
-                      WIDE ? tiled(128, 128, 0.9, 1.0, 1.5) : tiled(128, 128, 0.47, 0.55, 1.5),
-                      WIDE ? tiled(128, 128, 1.0, 0.9, 1.3) : tiled(128, 128, 0.53, 0.475, 1.3),
-                      WIDE ? tiled(128, 256, 1.6, 1.9, 3.8) : tiled(128, 256, 0.8, 0.99, 3.8),
+                      WIDE ? tiled(64, 128, 0.7, 0.53, 0.4) : tiled(64, 128, 0.34, 0.296, 0.4),
+                      WIDE ? tiled(128, 128, 1.02, 1.05, 1.5) : tiled(128, 128, 0.47, 0.55, 1.5),
+                      WIDE ? tiled(128, 128, 1.0, 0.87, 1.7) : tiled(128, 128, 0.53, 0.475, 1.3),
+                      WIDE ? tiled(128, 256, 1.6, 1.8, 5.) : tiled(128, 256, 0.8, 0.99, 3.8),
                       WIDE ? HUGE_VAL : tiled(256, 256, 1.22, 1.55, 10.)};
   const auto least = std::min_element(std::begin(t), std::end(t));
   DIGA_CHECK_ARG(*least < HUGE_VAL, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)p.M, p.N);
