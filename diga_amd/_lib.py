@@ -94,6 +94,8 @@ SIGNATURES = {
     "diga_grouped_matmul_fp8": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i, _vp, _i, _i64, _i64, _i, _i, _vp]),
     "diga_matmul_fp8_f32": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _vp]),
     "diga_grouped_matmul_fp8_f32": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i, _vp, _i64, _i64, _i, _i, _vp]),
+    "diga_matmul_use_tile": (_i, [_i]),
+    "diga_matmul_tile_of": (_i, [_i, _i, _i, _i64, _i64, _i, _i]),
     "diga_grouped_matmul": (_i, [_vp, _i64, _i64, _i, _vp, _vp, _i64, _i64, _vp, _i, _vp, _i, _i64, _i64, _i, _i, _vp]),
     "diga_nhwc_bf16_to_nchw_f32": (_i, [_vp, _vp, _i, _i, _i, _vp]),
     "diga_nchw_f32_to_nhwc_bf16": (_i, [_vp, _vp, _i, _i, _i, _vp]),

@@ -698,8 +698,11 @@ void launch_few(MatmulParams p, hipStream_t s) {
 // A launch has fewer than 2^32 threads: tiles that would need 2^23 blocks of 512 are left out.
 constexpr int64_t MAX_BLOCKS = ((int64_t)1 << 23) - 1;
 
+thread_local int asked_tile = -1;                          // diga_matmul_use_tile
+
+// index of the tile, -1 where none fits one launch
 template <int KIND, bool GROUPED>
-int launch(const char* who, const MatmulParams& p, hipStream_t s) {
+int choose(const MatmulParams& p) {
   constexpr bool WIDE = KIND == KIND_FP8_WIDE;
   const double groups = GROUPED ? (double)std::min<int64_t>(p.E, p.M) : 1., avg = (double)p.M / groups;
   const double once = ((double)p.xrows + groups * p.N) * p.Kb / 4.9e6;
@@ -723,14 +726,21 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
                       WIDE ? tiled(128, 128, 1.0, 0.87, 1.7) : tiled(128, 128, 0.53, 0.475, 1.3),
                       WIDE ? tiled(128, 256, 1.6, 1.8, 5.) : tiled(128, 256, 0.8, 0.99, 3.8),
                       WIDE ? HUGE_VAL : tiled(256, 256, 1.22, 1.55, 10.)};
-  const auto least = std::min_element(std::begin(t), std::end(t));
-  DIGA_CHECK_ARG(*least < HUGE_VAL, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)p.M, p.N);
+  static_assert(std::size(t) == DIGA_MATMUL_TILES);
+  const auto least = asked_tile >= 0 ? t + asked_tile : std::min_element(std::begin(t), std::end(t));
+  return *least < HUGE_VAL ? (int)(least - t) : -1;
+}
+
+template <int KIND, bool GROUPED>
+int launch(const char* who, const MatmulParams& p, hipStream_t s) {
+  const int tile = choose<KIND, GROUPED>(p);
+  DIGA_CHECK_ARG(tile >= 0, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)p.M, p.N);
   const int64_t size = p.out_type == DIGA_FP32 ? 4 : 2;
   DIGA_CHECK_ARG(!rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.x, p.rows ? p.xrows : p.M, p.ldx, p.Kb), "%s: the output lies on the left rows", who);
   DIGA_CHECK_ARG(!(p.E == 1 ? rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.w, p.N, p.ldw, p.Kb)
                             : rows_meet(p.out, p.M, p.ldo * size, p.N * size, p.w, p.E, p.wstride, (p.N - 1) * p.ldw + p.Kb)),
                  "%s: the output lies on the weights", who);
-  switch (least - t) {
+  switch (tile) {
     case 0: launch_few<KIND, 2, 1, 2, GROUPED>(p, s); break;
     case 1: launch_few<KIND, 2, 2, 2, GROUPED>(p, s); break;
     case 2: launch_few<KIND, 4, 2, 2, GROUPED>(p, s); break;
@@ -743,7 +753,7 @@ int launch(const char* who, const MatmulParams& p, hipStream_t s) {
     case 9: launch_tile<KIND, 128, 128, 2, 2, 2, GROUPED>(p, s); break;
     case 10: launch_tile<KIND, 128, 256, 2, 4, 2, GROUPED>(p, s); break;
     default:                                               // (its wide form would take more than 256 registers)
-      if constexpr (!WIDE) launch_tile<KIND, 256, 256, 2, 4, 2, GROUPED>(p, s);
+      if constexpr (KIND != KIND_FP8_WIDE) launch_tile<KIND, 256, 256, 2, 4, 2, GROUPED>(p, s);
       break;
   }
   DIGA_CHECK_LAUNCH(who);
@@ -861,4 +871,28 @@ extern "C" int diga_grouped_matmul(const void* x, int64_t ldx, int64_t x_rows, i
   p.M = T, p.xrows = x_rows, p.N = N, p.Kb = 2 * K, p.nk = cdiv(2 * (int64_t)K, 128), p.E = groups, p.out_type = out_type;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return type == DIGA_BF16 ? launch<KIND_BF16, true>(who, p, s) : launch<KIND_FP16, true>(who, p, s);
+}
+
+extern "C" int diga_matmul_use_tile(int tile) {
+  DIGA_CHECK_ARG(tile >= -1 && tile < DIGA_MATMUL_TILES, "diga_matmul_use_tile: tile %d (-1 .. %d)", tile, DIGA_MATMUL_TILES - 1);
+  asked_tile = tile;
+  return DIGA_OK;
+}
+
+extern "C" int diga_matmul_tile_of(int type, int out_type, int groups, int64_t M, int64_t x_rows, int N, int K) {
+  const char* who = "diga_matmul_tile_of";
+  DIGA_CHECK_ARG(type == DIGA_BF16 || type == DIGA_FP16 || type == DIGA_E4M3, "%s: unknown type %d", who, type);
+  DIGA_CHECK_ARG(groups >= (type == DIGA_E4M3 ? 0 : 1) && groups <= MAX_GROUPS, "%s: %d groups", who, groups);
+  const int size = type == DIGA_E4M3 ? 1 : 2;
+  DIGA_CHECK_ARG(M >= 1 && M <= MAX_M && x_rows >= 1 && x_rows <= MAX_M && N >= 1 && N <= MAX_N && K >= 1 && K <= MAX_ROW / size, "%s: M=%lld, %lld left rows, N=%d, K=%d", who,
+                 (long long)M, (long long)x_rows, N, K);
+  MatmulParams p{};
+  p.M = M, p.xrows = x_rows, p.N = N, p.Kb = K * size, p.nk = cdiv(p.Kb, 128), p.E = groups ? groups : 1;
+  int tile;
+  if (type == DIGA_BF16) tile = choose<KIND_BF16, true>(p);
+  else if (type == DIGA_FP16) tile = choose<KIND_FP16, true>(p);
+  else if (out_type == DIGA_FP32) tile = groups ? choose<KIND_FP8_WIDE, true>(p) : choose<KIND_FP8_WIDE, false>(p);
+  else tile = groups ? choose<KIND_FP8, true>(p) : choose<KIND_FP8, false>(p);
+  DIGA_CHECK_ARG(tile >= 0, "%s: M=%lld x N=%d has too many tiles for one launch", who, (long long)M, N);
+  return tile;
 }

@@ -36,6 +36,7 @@ extern "C" {
 #define DIGA_BF16 0
 #define DIGA_FP16 1
 #define DIGA_FP32 2
+#define DIGA_E4M3 3
 
 #define DIGA_MAX_TAPS 18
 #define DIGA_NUM_CLASSES_MAX 32
@@ -475,6 +476,13 @@ int diga_grouped_matmul_fp8_f32(const void* x, int64_t ldx, int64_t x_rows, cons
 int diga_grouped_matmul(const void* x, int64_t ldx, int64_t x_rows, int type, const int32_t* rows, const void* w,
                         int64_t ldw, int64_t w_stride, const int32_t* offsets, int groups, void* out, int out_type,
                         int64_t ldo, int64_t T, int N, int K, void* stream);
+/* For tests and measurements of the products.  Tiles, rows x weight rows: 0..6 with K steps dealt to 8 waves: 16x16, 16x32, 32x32, 48x32, 32x64,
+ * 48x64, 64x64; 7.. with both operands shared: 64x128, 128x128 of 8 waves, 128x128 of 4, 128x256, 256x256 (not for fp32 outputs of 8-bit products).
+ * diga_matmul_use_tile: the calling thread's products take this tile from now on, -1: by the rule; a product that the tile does not fit is refused.
+ * diga_matmul_tile_of: the tile of a product (type: of its operands; groups 0: dense, e4m3 only); launches nothing. */
+#define DIGA_MATMUL_TILES 12
+int diga_matmul_use_tile(int tile);
+int diga_matmul_tile_of(int type, int out_type, int groups, int64_t M, int64_t x_rows, int N, int K);
 
 /* Layout helpers for the Python-visible API (net(x, feat=True) returns NCHW fp32, adaptseg:188). */
 int diga_nhwc_bf16_to_nchw_f32(const void* in, float* out, int B, int HW, int C, void* stream);
