@@ -99,10 +99,6 @@ __device__ __forceinline__ f32x4 mfma_wide(const Wide& a, const Wide& b) {
   for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
   return c;
 }
-template <typename V>
-__device__ __forceinline__ i32x8 join_pair(const V& lo, const V& hi) {
-  return __builtin_shufflevector(__builtin_bit_cast(i32x4, lo), __builtin_bit_cast(i32x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
-}
 __device__ __forceinline__ i32x8 read_pair(const char* lo, const char* hi) {
   return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(lo), *reinterpret_cast<const i32x4*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
 }
