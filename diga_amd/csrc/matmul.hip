@@ -814,7 +814,7 @@ static int check_groups(const char* who, const int32_t* offsets, int groups, con
   DIGA_CHECK_ARG(T == 0 || offsets, "%s: null pointer", who);
   DIGA_CHECK_ARG(rows ? (T == 0 || x_rows > 0) : x_rows >= T, "%s: %lld left rows for %lld output rows", who, (long long)x_rows, (long long)T);
   DIGA_CHECK_ARG(!rows || x_rows <= 1 || ldx_bytes >= row_bytes, "%s: gathered rows of %lld bytes lie %lld bytes apart", who, (long long)row_bytes, (long long)ldx_bytes);
-  DIGA_CHECK_ARG(!rows || x_rows * ldx_bytes <= 0xffffffffll, "%s: rows are gathered from at most 4 GiB (%lld rows of %lld bytes)", who, (long long)x_rows, (long long)ldx_bytes);
+  DIGA_CHECK_ARG(!rows || (ldx_bytes <= 0xffffffffll && x_rows * ldx_bytes <= 0xffffffffll), "%s: rows are gathered from at most 4 GiB (%lld rows of %lld bytes)", who, (long long)x_rows, (long long)ldx_bytes);
   DIGA_CHECK_ARG(groups == 1 || w_stride >= (int64_t)(N - 1) * ldw, "%s: weight matrices overlap", who);
   return DIGA_OK;
 }

@@ -65,3 +65,11 @@ def test_norm_refuses_a_sum_written_across_its_inputs(change):
              stream=None)
     with pytest.raises(DigaError, match="lies across"):
         _lib.call("diga_rms_norm_fp8", *{**a, **change}.values())
+
+
+@pytest.mark.parametrize("ldx, x_rows", [(1 << 62, 4), (1 << 32, 1), (1 << 61, 8), ((1 << 32) - 16, 2)])
+def test_gathered_rows_beyond_4_gib_are_refused_whatever_their_product_wraps_to(ldx, x_rows):
+    a = dict(x=A, ldx=ldx, x_rows=x_rows, xs=A, ssm=1, ssb=4, rows=A, w=2 * A, ldw=256, w_stride=64 * 256, ws=A, offsets=A, groups=2, out=3 * A, out_type=0, ldo=64,
+             T=1, N=64, K=256, stream=None)
+    with pytest.raises(DigaError, match="at most 4 GiB"):
+        _lib.call("diga_grouped_matmul_fp8", *a.values())
