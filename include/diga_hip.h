@@ -435,9 +435,12 @@ int diga_nhwc_f32_to_nchw_f32(const float* in, float* out, int B, int HW, int C,
  * side, so scale_stride_m = 1 is its fast layout.  Row strides (ld*) count elements.  M = 0 rows: nothing is launched.
  * ------------------------------------------------------------------------------------------ */
 /* h = x (+ residual); y = h * weight / sqrt(mean(h^2) + eps), all in fp32; per row and block of 128 columns
- * scale = max(max|y|, 2^-100) / 448, q = e4m3(y / scale) (nearest even).  With a residual, h is also written to residual_out,
- * rounded to `type`; residual_out may be x or residual themselves (same stride), and is refused where it lies across them or the weight otherwise.  A NaN of y stays at its place; the row's scales
- * are those of its numbers.  x, residual, residual_out: `type`, weight [N]: weight_type.  N <= DIGA_RMS_NORM_MAX_N. */
+ * scale = max(max|y|, 2^-100) / 448, q = e4m3(y * (1 / scale)) (nearest even; 1 / scale is rounded, so a y within 2^-22 of a tie of y / scale may take
+ * the other neighbour).  An infinite y makes its block's scale infinite, itself NaN and the block's other values 0 (whose value, 0 * scale, is NaN).
+ * A NaN of y stays at its place; the row's scales are those of its numbers.
+ * The squares are summed in fp32: a row whose sum passes 2^128 (values about 2^64) comes out as zeros, one below 2^-126 with eps = 0 as NaN.
+ * With a residual, h is also written to residual_out, rounded to `type`; residual_out may be x or residual themselves (same stride), and is
+ * refused where it lies across them or the weight otherwise.  x, residual, residual_out: `type`, weight [N]: weight_type.  N <= DIGA_RMS_NORM_MAX_N. */
 #define DIGA_RMS_NORM_MAX_N 65536
 int diga_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, int type, const void* weight,
                       int weight_type, float eps, int64_t M, int N, void* q, int64_t ldq, float* scale,
@@ -449,9 +452,11 @@ int diga_silu_mul_fp8(const void* x, int64_t ldx, int type, int64_t M, int N, vo
 int diga_quantize_fp8(const void* x, int64_t ldx, int type, int64_t M, int N, void* q, int64_t ldq, float* scale,
                       int64_t scale_stride_m, int64_t scale_stride_b, void* stream);
 /* out[m][n] = sum_b x_scale[m][b] * w_scale[n / 128][b] * sum_{k in block b} x[m][k] * w[n][k], fp32 sums over the blocks, rounded once to
- * out_type (DIGA_BF16 or DIGA_FP16: the matrix pipe adds 8 e4m3 products with 13 bits below the largest, 2e-5 .. 5e-5 of a result, which
- * would not make a 32-bit one).  x: e4m3 [M][K]; w: e4m3 [N][K]; w_scale: fp32 [ceil(N/128)][ceil(K/128)]; out [M][N].
- * x and w rows start at multiples of 16 bytes (base and stride); a row's bytes up to K rounded up to 16 must be readable, what they
+ * out_type (DIGA_BF16 or DIGA_FP16: the matrix pipe cuts 8 consecutive products 13 bits below the largest of them, at most 2^-10 of the sum over
+ * such groups of their largest |product|, 1.5e-5 of the result in the 2-norm for normal operands; that would not make a 32-bit output).  The
+ * product of a block's two scales is taken first, in fp32: where it passes 2^128 the block is infinite or NaN.
+ * x: e4m3 [M][K]; w: e4m3 [N][K]; w_scale: fp32 [ceil(N/128)][ceil(K/128)]; out [M][N].
+ * x and w rows start at multiples of 16 bytes (base and stride, at most 8 MiB apart); a row's bytes up to K rounded up to 16 must be readable, what they
  * hold does not matter.  out may not lie on x or w.  No scratch memory. */
 int diga_matmul_fp8(const void* x, int64_t ldx, const float* x_scale, int64_t x_scale_stride_m,
                     int64_t x_scale_stride_b, const void* w, int64_t ldw, const float* w_scale, void* out, int out_type,
