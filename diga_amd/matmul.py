@@ -20,7 +20,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version as _written      # a tensor written in place: a backward that saved it has to notice
 
 from ._lib import DigaError, check, load
@@ -43,7 +43,6 @@ _HALVES = {torch.bfloat16: 0, torch.float16: 1}
 _E4M3 = {E4M3: 0}
 _stream_of = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
-_fwd_grad_enabled = torch._C._is_fwd_grad_enabled
 _empty, _strided = torch.empty, torch.empty_strided
 
 
@@ -79,6 +78,7 @@ def _device(who, *tensors):
     index = tensors[0].get_device()
     if index < 0:
         raise DigaError(f"{who}: tensors must be on the GPU: there is no CPU fallback")
+    tangents = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()      # (no tensor has one outside a level)
     for t in tensors:
         if t is not None:
             if t.get_device() != index:
@@ -87,7 +87,7 @@ def _device(who, *tensors):
                 raise DigaError(f"{who}: a tensor's values are held negated: pass its resolve_neg()")
             if t.requires_grad and torch.is_grad_enabled():
                 raise DigaError(f"{who} has no backward pass: call it under torch.no_grad() or on detached tensors")
-            if _fwd_grad_enabled() and unpack_dual(t).tangent is not None:
+            if tangents and forward_ad.unpack_dual(t).tangent is not None:
                 raise DigaError(f"{who} has no derivative: a tensor carries a tangent, which would be dropped: pass it without")
     return index
 
@@ -261,11 +261,13 @@ def matmul_fp8(xq, xs, wq, ws, out_dtype=torch.bfloat16, out=None):
     _check_out(who, out, m, n, out_dtype)
     _check_wide(who, out_dtype, xq)
     index = _device(who, xq, xs, wq, ws, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty((m, n), dtype=out_dtype, device=xq.device)
     entry, kind = _fp8_entry(out_dtype, _matmul, _matmul_f32)
     entry(index, xq.data_ptr(), ldx, xs.data_ptr(), sm, sb, wq.data_ptr(), ldw, ws.data_ptr(), out.data_ptr(), *kind, out.stride(0), m, n, k)
-    _written(out)
+    if given:
+        _written(out)
     return out
 
 
@@ -299,12 +301,14 @@ def grouped_matmul_fp8(xq, xs, wq, ws, offsets, rows=None, out_dtype=torch.bfloa
     _check_out(who, out, t, n, out_dtype)
     _check_wide(who, out_dtype, xq)
     index = _device(who, xq, xs, wq, ws, offsets, rows, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty((t, n), dtype=out_dtype, device=xq.device)
     entry, kind = _fp8_entry(out_dtype, _grouped_fp8, _grouped_fp8_f32)
     entry(index, xq.data_ptr(), ldx, xr, xs.data_ptr(), sm, sb, rows.data_ptr() if rows is not None else None, wq.data_ptr(), ldw,
           we, ws.data_ptr(), offsets.data_ptr(), e, out.data_ptr(), *kind, out.stride(0), t, n, k)
-    _written(out)
+    if given:
+        _written(out)
     return out
 
 
@@ -318,9 +322,11 @@ def grouped_matmul(x, w, offsets, rows=None, out_dtype=None, out=None):
     xr, k, e, n, t, we, ldx, ldw = _groups(who, x, w, offsets, rows, _HALVES, 8)
     _check_out(who, out, t, n, out_dtype)
     index = _device(who, x, w, offsets, rows, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty((t, n), dtype=out_dtype, device=x.device)
     _grouped(index, x.data_ptr(), ldx, xr, _HALVES[x.dtype], rows.data_ptr() if rows is not None else None, w.data_ptr(), ldw, we,
              offsets.data_ptr(), e, out.data_ptr(), _TYPES[out_dtype], out.stride(0), t, n, k)
-    _written(out)
+    if given:
+        _written(out)
     return out
